@@ -62,18 +62,24 @@ def attend(q: torch.Tensor, p: torch.Tensor, k: torch.Tensor, v: torch.Tensor, s
     -> (out float64 [T, H, D], bound [T, H, D]).
 
     The bound: a score is a sum of D products in fp32 and two more roundings, off by at most
-    (D + 2) 2^-24 sum |q k| scale, and the difference to the maximum, the exponential (one unit in
-    the last place) and the base change add 2^-22 (1 + |s - max|); a probability's relative error d
-    enters numerator and denominator.  P is rounded once, to bf16 in the open block (2^-8) and to fp16
-    elsewhere (2^-11), the output to bf16 once; sums over n positions and split states add
-    (n + 64) 2^-24 of the magnitudes.
+    (D + 2) 2^-24 sum |q k| scale; a query element below 2^-31 of its row's largest is rounded to steps
+    of 2^-38 of that (fp16 of the scaled row), 2^-39 max |q| |k| each.  The difference to the maximum, the
+    exponential (one unit in the last place), the base change and the logarithm in the exponent add
+    2^-19 + 2^-22 |s - max|.  A probability's relative error d enters numerator and denominator.
 
-    fp16 has steps of 2^-24 below 2^-14.  What is rounded is x = P v_scale f, f a power of two that only
-    falls and starts, and is set again, so that v_scale f lies in [2^6, 2^7): 1 / f <= 2^-6 times the
-    largest v_scale.  Half a step of x, 2^-25, is 2^-25 |code| / f <= 2^-31 max |v| in the sum, as
-    |code| v_scale <= amax; over n positions, with the denominator at least 1 (P is relative to a
-    reference at or below the maximum), n 2^-31 max |v|.  (f is held below 2^100: blocks of values below
-    2^-94 lose at most 2^-125 |code| a position.)"""
+    P is rounded once for the product, to bf16 in the open block (2^-8) and to fp16 elsewhere (2^-11),
+    and the denominator may be the sum of the rounded ones.  sum w_i (1 + r_i) v_i / sum w_i (1 + r_i) is then
+    off by at most sum w_i |r_i| (|v_i| + |out|).
+
+    fp16 has steps of 2^-24 below 2^-14.  What is rounded is P g with g >= 2^3, P relative to a reference
+    that is at or below the row's maximum: half a step is 2^-25 / g <= 2^-28 in units in which the
+    denominator is at least 1, so a seen position's value enters wrong by at most 2^-28 |v| and the
+    denominator by 2^-28.
+
+    Sums over n positions and split states add (n + 64) 2^-24 of the magnitudes, the output is rounded to
+    bf16 once.  Sums are held in units of at least 2^-32, so that fp32's smallest step, 2^-149, is 2^-117.
+
+    Only values that a row sees are in its bound, but they have to be numbers throughout."""
     T, H, D = q.shape
     KVH, n, _ = k.shape
     at = torch.arange(n)
@@ -93,13 +99,15 @@ def attend(q: torch.Tensor, p: torch.Tensor, k: torch.Tensor, v: torch.Tensor, s
         m = torch.where(torch.isinf(m), torch.zeros_like(m), m)
         e = torch.exp(s - m)
         gap = torch.where(seen, (s - m).abs(), torch.zeros_like(s))
-        d = (D + 2) * 2.0 ** -24 * mag + 2.0 ** -22 * (1 + gap)
+        flushed = 2.0 ** -39 * qq.abs().amax(1, keepdim=True) * kk.abs().sum(1) * abs(scale)
+        d = (D + 2) * 2.0 ** -24 * mag + flushed.masked_fill(~seen, 0.0) + 2.0 ** -19 + 2.0 ** -22 * gap
         d = d + d.masked_fill(~seen, 0.0).amax(1, keepdim=True)            # the maximum is off as well
         l = e.sum(1, keepdim=True)
         w = torch.where(rows[:, None], e / torch.where(l > 0, l, torch.ones_like(l)), torch.zeros_like(e))
         out[:, h] = w @ vv
         spread = (w * d) @ vv.abs() + (w * d).sum(1, keepdim=True) * (w @ vv.abs())
-        vmax = vv.abs().max() if n else 0.0
-        bound[:, h] = (1.01 * (spread + n * 2.0 ** -31 * vmax) + (HALF[torch.bfloat16] + (n + 64) * 2.0 ** -24) * (w @ vv.abs())
-                       + HALF[torch.bfloat16] * out[:, h].abs() * 1.01 + n * 2.0 ** -116)
+        mean, o = w @ vv.abs(), out[:, h].abs()
+        small = 2.0 ** -28 * (seen.double() @ vv.abs() + seen.sum(1, keepdim=True) * o)
+        bound[:, h] = 1.01 * (spread + small + HALF[torch.bfloat16] * (mean + o) + HALF[torch.bfloat16] * o) + (
+            (n + 64) * 2.0 ** -24 * mean + n * 2.0 ** -116)
     return out, bound

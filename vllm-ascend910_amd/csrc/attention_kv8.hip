@@ -12,11 +12,11 @@
 //           l' = l a + sum P,  O' = O a + f16(P * v_scale * f) . codes
 //   output  bf16(O / (f l)); zeros for a row that attends to nothing
 // so that neither operand is dequantised element by element: a block's scales enter with
-// ck and with the exponent.  f is a power of two that keeps v_scale * f near 2^6, with P
-// (up to 2^4) in the upper half of fp16's range: P is then rounded to 11 bits, where bf16
-// would leave 8 (relative error of a step's output 2.5e-3 with bf16 P, 1.7e-3 with fp16,
-// of which the output's own rounding is 1.7e-3).  Below 2^-20 P has steps of 2^-30.  The
-// query loses bits only below 2^-38 of its largest element.  The open block's keys and
+// ck and with the exponent.  f is a power of two that keeps v_scale * f in [2^3, 2^11],
+// with P (up to 2^4) in the upper half of fp16's range: P is then rounded to 11 bits, where
+// bf16 would leave 8 (relative error of a step's output 2.5e-3 with bf16 P, 1.7e-3 with
+// fp16, of which the output's own rounding is 1.7e-3), below 2^-17 to steps of 2^-27 at most.
+// The query loses bits only below 2^-31 of its largest element.  The open block's keys and
 // values are the bf16 ones of the tails, and their products bf16's.
 #include <algorithm>
 #include <cmath>
@@ -95,37 +95,69 @@ __device__ __forceinline__ float query_f16(const uint4 (&q)[D / 32], f16x8 (&qh)
 }
 
 // The units of a wave's O, which holds f times the sum (f a power of two, the same for
-// all rows of the wave; 0 before the first chunk of codes, where O holds the sum itself).
+// all rows of the wave; 0 before the first chunk that sets it: O holds the sum itself).
 // One chunk's V scale in them:
 struct VScale {
     float g;       // v_scale * f
     float lg;      // log2(g)
     float inv;     // 1 / g
-    bool plain;    // g is a number in [2^-60, 2^11]: 2^(s - m + lg) stays a normal float and an fp16
+    bool plain;    // g is in [kLeastG, kMostG]
 };
 
 // A row's m is the reference of its exponents, not quite its maximum: it is raised to the
 // maximum only where that has passed it by 2^kSlack, so that after the first chunks O is
 // hardly ever rescaled (in tiles of sixteen rows some row's maximum moves in half of the
 // first 64 chunks).  P is then at most 2^kSlack, and g at most 2^(15 - kSlack).
+//
+// fp16 has steps of 2^-24 below 2^-14: P is off by 2^-25 / g there.  The denominator is the
+// sum of the same rounded P, at least 1 over all of a row's positions, so with g from 2^3 on
+// a position takes at most 2^-28 from it, and as much of its own value from the product
+// (2^-13 over 32768 positions; an output's rounding is 2^-9).  f is set to bring g into
+// [2^9, 2^10): later blocks may be twice as large before O is rescaled, and 64 times as
+// small before they leave the plain way.
 constexpr float kSlack = 4.0f;
+constexpr float kLeastG = 0x1p3f, kMostG = 0x1p11f;
 
-// `rescale(x)`: O takes the factor x, a power of two.
+// The exponent of a number (-1 for zero, infinities and NaN), by a vector instruction: from
+// its bits the compiler takes scales to scalar registers, and waits for a chunk's loads as
+// soon as they are requested (a windowed step of 32 sequences 34 us instead of 27).
+__device__ __forceinline__ int exponent(float x) { return __builtin_amdgcn_frexp_expf(x) - 1; }
+
+// `rescale(x)`: O takes the factor x, a power of two.  f is set by the first block whose
+// scale is a number from 2^-23 on (one of zeros, or of values that small, says nothing of
+// the others) and set again, lower, where a larger one comes.  It stays in [2^-32, 2^32], so
+// that f times a sum stays inside fp32's range for rows that do not see the block.
 template <class F>
 __device__ __forceinline__ VScale v_scale(float vs, float& f, F rescale) {
     VScale v;
-    v.g = vs * f;
-    if (f == 0.0f || v.g > 0x1p11f) {
-        const int e = static_cast<int>((__float_as_uint(vs) >> 23) & 255) - 127;   // 128 for NaN
-        const float fn = __uint_as_float(static_cast<uint32_t>(127 + max(min(6 - e, 100), -120)) << 23);
-        rescale(f == 0.0f ? fn : fn / f);
-        f = fn;
-        v.g = vs * f;
+    v.g = f == 0.0f ? vs : vs * f;
+    if (f == 0.0f || v.g > kMostG) {
+        const float fn = ldexpf(1.0f, max(9 - exponent(vs), -32));
+        if (vs >= 0x1p-23f && vs < INFINITY && fn != f) {
+            rescale(f == 0.0f ? fn : fn / f);
+            f = fn;
+            v.g = vs * fn;
+        }
     }
-    v.plain = v.g >= 0x1p-60f && v.g <= 0x1p11f;      // false for NaN
+    v.plain = v.g >= kLeastG && v.g <= kMostG;        // false for NaN
     v.lg = __builtin_amdgcn_logf(v.g);
     v.inv = __builtin_amdgcn_rcpf(v.g);                // off by one unit in the last place at most
     return v;
+}
+
+// A chunk whose scale is not plain (values of quite another size than those of the blocks
+// before, zeros, NaN).  A row that sees some of it takes its O times 2^k for that chunk's
+// product and back after it: k brings v_scale * f * 2^k into [2^9, 2^10) where that leaves
+// O below 2^120 (beyond, the chunk is below 2^-90 of what the row holds) and the units at
+// most 2^100.
+// P's factor, v_scale * f * 2^k, is returned.  largest: of the row's O; unit(k): O takes the
+// factor 2^k.
+template <class F>
+__device__ __forceinline__ float own_unit(int& k, bool sees, float vs, float f, float largest, F unit) {
+    const int fe = f == 0.0f ? 0 : exponent(f);
+    k = sees && vs < INFINITY ? min(min(9 - exponent(vs), 100) - fe, 119 - exponent(largest)) : 0;
+    unit(k);
+    return sees ? ldexpf(vs, fe + k) : 0.0f;
 }
 
 // The chunks that any row of a tile attends to: the first nsink, then wlo .. wlo + n - nsink - 1.
@@ -181,6 +213,25 @@ __device__ __forceinline__ void scale_o(RowState<D>& st, float x) {
         for (int e = 0; e < 4; ++e) st.o[dt][e] = st.o[dt][e] * x;
 }
 
+// O times 2^k; the largest element of a row's O.
+template <int D>
+__device__ __forceinline__ void shift_o(RowState<D>& st, int k) {
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) st.o[dt][e] = ldexpf(st.o[dt][e], k);
+}
+
+template <int D>
+__device__ __forceinline__ float largest_o(const RowState<D>& st) {
+    float x = 0.0f;
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x = fmaxf(x, fabsf(st.o[dt][e]));
+    return row_reduce(x, [](float a, float b) { return fmaxf(a, b); });
+}
+
 // The scores that a row does not see taken as -inf.
 __device__ __forceinline__ void hide(f32x4 (&sc)[4], uint32_t seen) {
 #pragma unroll
@@ -191,22 +242,22 @@ __device__ __forceinline__ void hide(f32x4 (&sc)[4], uint32_t seen) {
 }
 
 // The softmax update of one chunk from its raw scores: m and l of the state, P^T (times the
-// chunk's V scale) as the B operands of the chunk's two key blocks, and where a row's
-// reference is raised `rescale(alpha)`: O takes the factor alpha.  ck >= 0: what a raw
-// score is multiplied by.
+// chunk's V scale; where that is not plain, times what `factor(sees)` gives) as the B
+// operands of the chunk's two key blocks, and where a row's reference is raised
+// `rescale(alpha)`: O takes the factor alpha.  ck >= 0: what a raw score is multiplied by.
 //
 // Where every row's maximum is a number below 2^12 the exponent is one fused multiply-add
 // of the raw score, s ck + (lg - m): lg - m is off by at most 2^-13, the relative error
 // of all of the row's probabilities in the chunk, 2^-18 at maxima below 100.  Elsewhere
-// (maxima beyond, no position seen yet, NaN, a V scale far below the earlier ones) the
+// (maxima beyond, no position seen yet, NaN, a V scale that is not plain) the
 // exponent is the difference of two rounded products, exactly 0 for the largest.
 //
 // On the first way the sum of P, like the output, is the matrix unit's (sum_p: P^T times
 // ones, of which the row's l takes linv): the sixteen additions and the lane reduction
 // were a quarter of the vector instructions.  On the other l is complete, linv 0.
-template <class E, class F>
+template <class E, class F, class G>
 __device__ __forceinline__ void softmax8(float& m, float& l, float& linv, E (&pop)[2], f32x4 (&sc)[4], float ck, const VScale& v,
-                                         F rescale) {
+                                         F rescale, G factor) {
 #pragma clang fp contract(off)
     float top = -INFINITY;
 #pragma unroll
@@ -242,8 +293,6 @@ __device__ __forceinline__ void softmax8(float& m, float& l, float& linv, E (&po
         const float mx = vmax(m, top);
         const float mz = mx == -INFINITY ? 0.0f : mx;    // nothing seen yet: everything stays 0
         const float alpha = m != -INFINITY ? __builtin_amdgcn_exp2f(m - mz) : 1.0f;
-        // a row that sees nothing of the chunk takes nothing from it, whatever its scale
-        const float g = top == -INFINITY ? 0.0f : v.g;
         float ls = 0.0f;
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt)
@@ -251,12 +300,17 @@ __device__ __forceinline__ void softmax8(float& m, float& l, float& linv, E (&po
             for (int e = 0; e < 4; ++e) {
                 sc[kt][e] = __builtin_amdgcn_exp2f(sc[kt][e] - mz);
                 ls = ls + sc[kt][e];
-                sc[kt][e] = sc[kt][e] * g;
             }
         l = fmaf(l, alpha, row_reduce(ls, [](float a, float b) { return a + b; }));
         linv = 0.0f;
         m = mx;
         rescale(alpha);
+        // a row that sees nothing of the chunk takes nothing from it, whatever its scale
+        const float g = v.plain ? v.g : factor(top != -INFINITY);
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[kt][e] = sc[kt][e] * g;
     }
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -320,7 +374,11 @@ __device__ __forceinline__ void chunk_codes(CodeState<D>& st, const f16x8 (&qh)[
     float linv;
     f16x8 pop[2];
     hide(sc, seen);
-    softmax8(st.m, st.l, linv, pop, sc, ck * ks, v, [&](float x) __attribute__((always_inline)) { scale_o<D>(st, x); });
+    int k = 0;
+    softmax8(st.m, st.l, linv, pop, sc, ck * ks, v, [&](float x) __attribute__((always_inline)) { scale_o<D>(st, x); },
+             [&](bool sees) __attribute__((always_inline)) {
+                 return own_unit(k, sees, vs, st.f, largest_o<D>(st), [&](int n) { shift_o<D>(st, n); });
+             });
     const float sum = sum_p(pop);
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) {
@@ -332,6 +390,7 @@ __device__ __forceinline__ void chunk_codes(CodeState<D>& st, const f16x8 (&qh)[
     }
     st.l = fmaf(sum, linv, st.l);
     next_v();
+    if (__builtin_expect(!v.plain, 0)) shift_o<D>(st, -k);
     __builtin_amdgcn_sched_barrier(0);
 }
 
@@ -397,7 +456,8 @@ __device__ __forceinline__ void chunk_tail(RowState<D>& st, const TailLds<D>& t,
     float linv;
     bf16x8 pop[2];
     hide(sc, seen_bits(a, p_row, c0, j));
-    softmax8(st.m, st.l, linv, pop, sc, a.cs, VScale{1.0f, 0.0f, 1.0f, true}, [&](float x) __attribute__((always_inline)) { scale_o<D>(st, x); });
+    softmax8(st.m, st.l, linv, pop, sc, a.cs, VScale{1.0f, 0.0f, 1.0f, true}, [&](float x) __attribute__((always_inline)) { scale_o<D>(st, x); },
+             [](bool) { return 1.0f; });
     st.l = fmaf(sum_p(pop), linv, st.l);
     uint32_t in[2][4];
 #pragma unroll
@@ -628,7 +688,7 @@ __device__ __forceinline__ void chunk_completed(RowState<D>& st, const TailLds<D
     float linv;
     f16x8 pop[2];
     hide(sc, seen);
-    softmax8(st.m, st.l, linv, pop, sc, ck * scale.x, VScale{0x1p6f, 6.0f, 0x1p-6f, true}, [](float) {});
+    softmax8(st.m, st.l, linv, pop, sc, ck * scale.x, VScale{0x1p6f, 6.0f, 0x1p-6f, true}, [](float) {}, [](bool) { return 1.0f; });
     st.l = fmaf(sum_p(pop), linv, st.l);
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt)
@@ -1054,11 +1114,15 @@ __global__ __launch_bounds__(64 * kLoopWaves, 2) void attn8_loop_kernel(const At
         });
         f16x8 pop[RT][2];
         float linv[RT];
+        int k[RT] = {};
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
             if (masked) hide(sc[t], seen_bits(a, row(t).p, c0, j));
             softmax8(st[t].m, st[t].l, linv[t], pop[t], sc[t], ck[t] * ks, v,
-                     [&](float x) __attribute__((always_inline)) { scale_o<D>(st[t], x); });
+                     [&](float x) __attribute__((always_inline)) { scale_o<D>(st[t], x); },
+                     [&](bool sees) __attribute__((always_inline)) {
+                         return own_unit(k[t], sees, vs, st[0].f, largest_o<D>(st[t]), [&](int n) { shift_o<D>(st[t], n); });
+                     });
         }
         float sum[RT];
         __builtin_amdgcn_s_setprio(1);
@@ -1079,6 +1143,10 @@ __global__ __launch_bounds__(64 * kLoopWaves, 2) void attn8_loop_kernel(const At
         __builtin_amdgcn_s_setprio(0);
 #pragma unroll
         for (int t = 0; t < RT; ++t) st[t].l = fmaf(sum[t], linv[t], st[t].l);
+        if (__builtin_expect(!v.plain, 0)) {
+#pragma unroll
+            for (int t = 0; t < RT; ++t) shift_o<D>(st[t], -k[t]);
+        }
     };
     store(buf[0]);
     load(i0 + 1);
