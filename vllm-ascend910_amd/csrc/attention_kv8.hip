@@ -123,17 +123,19 @@ constexpr float kLeastG = 0x1p3f, kMostG = 0x1p11f;
 // soon as they are requested (a windowed step of 32 sequences 34 us instead of 27).
 __device__ __forceinline__ int exponent(float x) { return __builtin_amdgcn_frexp_expf(x) - 1; }
 
-// `rescale(x)`: O takes the factor x, a power of two.  f is set by the first block whose
-// scale is a number from 2^-23 on (one of zeros, or of values that small, says nothing of
-// the others) and set again, lower, where a larger one comes.  It stays in [2^-32, 2^32], so
-// that f times a sum stays inside fp32's range for rows that do not see the block.
-template <class F>
-__device__ __forceinline__ VScale v_scale(float vs, float& f, F rescale) {
+// `rescale(x)`: O takes the factor x, a power of two; `room()`: O has no element from 2^90 on
+// (an open block's values, taken first, may be there before f is set).  f is set by the
+// first block whose scale is a number from 2^-23 on (one of zeros, or of values that small,
+// says nothing of the others) and set again, lower, where a larger one comes.  It stays in
+// [2^-32, 2^32], so that f times a sum stays inside fp32's range for rows that do not see
+// the block.
+template <class F, class G>
+__device__ __forceinline__ VScale v_scale(float vs, float& f, F rescale, G room) {
     VScale v;
     v.g = f == 0.0f ? vs : vs * f;
     if (f == 0.0f || v.g > kMostG) {
         const float fn = ldexpf(1.0f, max(9 - exponent(vs), -32));
-        if (vs >= 0x1p-23f && vs < INFINITY && fn != f) {
+        if (vs >= 0x1p-23f && vs < INFINITY && fn != f && (f != 0.0f || room())) {
             rescale(f == 0.0f ? fn : fn / f);
             f = fn;
             v.g = vs * fn;
@@ -370,7 +372,8 @@ __device__ __forceinline__ void chunk_codes(CodeState<D>& st, const f16x8 (&qh)[
     __builtin_amdgcn_sched_barrier(0);
     next_k();
     __builtin_amdgcn_sched_barrier(0);
-    const VScale v = v_scale(vs, st.f, [&](float x) __attribute__((always_inline)) { scale_o<D>(st, x); });
+    const VScale v = v_scale(vs, st.f, [&](float x) __attribute__((always_inline)) { scale_o<D>(st, x); },
+                             [&]() __attribute__((always_inline)) { return __builtin_amdgcn_ballot_w64(largest_o<D>(st) >= 0x1p90f) == 0; });
     float linv;
     f16x8 pop[2];
     hide(sc, seen);
@@ -1111,7 +1114,7 @@ __global__ __launch_bounds__(64 * kLoopWaves, 2) void attn8_loop_kernel(const At
         const VScale v = v_scale(vs, st[0].f, [&](float x) __attribute__((always_inline)) {
 #pragma unroll
             for (int t = 0; t < RT; ++t) scale_o<D>(st[t], x);
-        });
+        }, []() { return true; });                       // the open block comes last here
         f16x8 pop[RT][2];
         float linv[RT];
         int k[RT] = {};
