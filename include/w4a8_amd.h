@@ -401,8 +401,9 @@ int w4a8_kv8_read(const void* k_codes, const void* vt_codes, const void* kv_scal
  * before).  q, out bf16 [B, T, H, D]; query head h*G + g reads KV head h, G = H / KVH.
  * The token at position p attends to the positions k <= p; with window > 0 only to those
  * with k > p - window or k < sinks.  Scores, softmax statistics and sums are fp32, the
- * probabilities are rounded for the product with V (to fp16 over a block's codes, to bf16
- * over the open block's values), a token that attends to nothing gives zeros.  `workspace`: w4a8_attention_kv8_workspace_bytes bytes.
+ * probabilities are rounded for the product with V (to fp16 over a block's codes, to the
+ * sum of two bf16 over the open block's values), a token that attends to nothing gives
+ * zeros.  `workspace`: w4a8_attention_kv8_workspace_bytes bytes.
  */
 int w4a8_attention_kv8(const void* q, const void* k_codes, const void* vt_codes, const void* kv_scale,
                        const void* k_tail, const void* vt_tail, int code_dtype, void* out, const void* pos,

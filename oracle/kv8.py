@@ -14,6 +14,7 @@ import torch
 BLOCK = 64
 TOP = {torch.int8: 127, torch.float8_e4m3fn: 448}
 HALF = {torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}   # half a step, relative to the value
+FP16 = 2.0 ** -11
 
 
 def round_e4m3(y: torch.Tensor) -> torch.Tensor:
@@ -67,7 +68,7 @@ def attend(q: torch.Tensor, p: torch.Tensor, k: torch.Tensor, v: torch.Tensor, s
     exponential (one unit in the last place), the base change and the logarithm in the exponent add
     2^-19 + 2^-22 |s - max|.  A probability's relative error d enters numerator and denominator.
 
-    P is rounded once for the product, to bf16 in the open block (2^-8) and to fp16 elsewhere (2^-11),
+    P is rounded once for the product, to fp16 (2^-11; the pair of bf16 over the open block leaves 2^-16),
     and the denominator may be the sum of the rounded ones.  sum w_i (1 + r_i) v_i / sum w_i (1 + r_i) is then
     off by at most sum w_i |r_i| (|v_i| + |out|).
 
@@ -108,6 +109,6 @@ def attend(q: torch.Tensor, p: torch.Tensor, k: torch.Tensor, v: torch.Tensor, s
         spread = (w * d) @ vv.abs() + (w * d).sum(1, keepdim=True) * (w @ vv.abs())
         mean, o = w @ vv.abs(), out[:, h].abs()
         small = 2.0 ** -28 * (seen.double() @ vv.abs() + seen.sum(1, keepdim=True) * o)
-        bound[:, h] = 1.01 * (spread + small + HALF[torch.bfloat16] * (mean + o) + HALF[torch.bfloat16] * o) + (
+        bound[:, h] = 1.01 * (spread + small + FP16 * (mean + o) + HALF[torch.bfloat16] * o) + (
             (n + 64) * 2.0 ** -24 * mean + n * 2.0 ** -116)
     return out, bound

@@ -14,10 +14,10 @@
 // so that neither operand is dequantised element by element: a block's scales enter with
 // ck and with the exponent.  f is a power of two that keeps v_scale * f in [2^3, 2^11],
 // with P (up to 2^4) in the upper half of fp16's range: P is then rounded to 11 bits, where
-// bf16 would leave 8 (relative error of a step's output 2.5e-3 with bf16 P, 1.7e-3 with
-// fp16, of which the output's own rounding is 1.7e-3), below 2^-17 to steps of 2^-27 at most.
-// The query loses bits only below 2^-31 of its largest element.  The open block's keys and
-// values are the bf16 ones of the tails, and their products bf16's.
+// bf16 would leave 8, below 2^-17 to steps of 2^-27 at most (relative error of a step's output
+// over 1000 positions 1.568e-3, of which the output's own rounding is 1.562e-3).  The query
+// loses bits only below 2^-31 of its largest element.  The open block's keys and values are
+// the bf16 ones of the tails, its products bf16's, with P as a pair of them.
 #include <algorithm>
 #include <cmath>
 
@@ -243,10 +243,10 @@ __device__ __forceinline__ void hide(f32x4 (&sc)[4], uint32_t seen) {
             sc[kt][e] = __uint_as_float(bit_select(bit_mask(seen, slot_pos(kt, 0, e)), __float_as_uint(sc[kt][e]), 0xff800000u));
 }
 
-// The softmax update of one chunk from its raw scores: m and l of the state, P^T (times the
-// chunk's V scale; where that is not plain, times what `factor(sees)` gives) as the B
-// operands of the chunk's two key blocks, and where a row's reference is raised
-// `rescale(alpha)`: O takes the factor alpha.  ck >= 0: what a raw score is multiplied by.
+// The softmax update of one chunk: its raw scores become P^T (times the chunk's V scale;
+// where that is not plain, times what `factor(sees)` gives), m and l of the state follow, and
+// where a row's reference is raised `rescale(alpha)`: O takes the factor alpha.  ck >= 0: what
+// a raw score is multiplied by.
 //
 // Where every row's maximum is a number below 2^12 the exponent is one fused multiply-add
 // of the raw score, s ck + (lg - m): lg - m is off by at most 2^-13, the relative error
@@ -257,9 +257,9 @@ __device__ __forceinline__ void hide(f32x4 (&sc)[4], uint32_t seen) {
 // On the first way the sum of P, like the output, is the matrix unit's (sum_p: P^T times
 // ones, of which the row's l takes linv): the sixteen additions and the lane reduction
 // were a quarter of the vector instructions.  On the other l is complete, linv 0.
-template <class E, class F, class G>
-__device__ __forceinline__ void softmax8(float& m, float& l, float& linv, E (&pop)[2], f32x4 (&sc)[4], float ck, const VScale& v,
-                                         F rescale, G factor) {
+template <class F, class G>
+__device__ __forceinline__ void softmax8(float& m, float& l, float& linv, f32x4 (&sc)[4], float ck, const VScale& v, F rescale,
+                                         G factor) {
 #pragma clang fp contract(off)
     float top = -INFINITY;
 #pragma unroll
@@ -314,6 +314,11 @@ __device__ __forceinline__ void softmax8(float& m, float& l, float& linv, E (&po
 #pragma unroll
             for (int e = 0; e < 4; ++e) sc[kt][e] = sc[kt][e] * g;
     }
+}
+
+// P^T as the B operands of a chunk's two key blocks.
+template <class E>
+__device__ __forceinline__ void operands_p(const f32x4 (&sc)[4], E (&pop)[2]) {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
         uint32_t w[4];
@@ -324,6 +329,14 @@ __device__ __forceinline__ void softmax8(float& m, float& l, float& linv, E (&po
         }
         pop[s] = __builtin_bit_cast(E, make_uint4(w[0], w[1], w[2], w[3]));
     }
+}
+
+// What the bf16 operands hi leave of P.  (An infinite or NaN P leaves nothing.)
+__device__ __forceinline__ void rest_p(f32x4 (&sc)[4], const bf16x8 (&hi)[2]) {
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[kt][e] = sc[kt][e] - static_cast<float>(hi[kt / 2][4 * (kt & 1) + e]);
 }
 
 // The sums of P^T's columns, each in every lane and element of its row: ones times P^T.
@@ -378,10 +391,11 @@ __device__ __forceinline__ void chunk_codes(CodeState<D>& st, const f16x8 (&qh)[
     f16x8 pop[2];
     hide(sc, seen);
     int k = 0;
-    softmax8(st.m, st.l, linv, pop, sc, ck * ks, v, [&](float x) __attribute__((always_inline)) { scale_o<D>(st, x); },
+    softmax8(st.m, st.l, linv, sc, ck * ks, v, [&](float x) __attribute__((always_inline)) { scale_o<D>(st, x); },
              [&](bool sees) __attribute__((always_inline)) {
                  return own_unit(k, sees, vs, st.f, largest_o<D>(st), [&](int n) { shift_o<D>(st, n); });
              });
+    operands_p(sc, pop);
     const float sum = sum_p(pop);
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) {
@@ -441,7 +455,10 @@ __device__ __forceinline__ void request_tail(TailLds<D>& t, const AttnKv8Args& a
 __device__ __forceinline__ void await_tail() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // The open block (positions c0 .. held - 1 hold values, the tail's other slots whatever
-// was there) into a row's state.  hidden: some of those positions are hidden from a row;
+// was there) into a row's state.  Its values are not fp16 numbers; P is the sum of two bf16
+// operands (2^-16), so that a short sequence is as precise as a long one: over 40 positions
+// the output is off by 1.87e-3 with one, 1.61e-3 with two, all of it its own rounding (a
+// step of one sequence 10.6 / 10.9 us).  hidden: some of those positions are hidden from a row;
 // an infinity or NaN among their values must not reach it through 0 * value.
 template <int D>
 __device__ __forceinline__ void chunk_tail(RowState<D>& st, const TailLds<D>& t, const uint4 (&q)[D / 32],
@@ -457,11 +474,32 @@ __device__ __forceinline__ void chunk_tail(RowState<D>& st, const TailLds<D>& t,
         __builtin_amdgcn_sched_barrier(0);   // one tile's operands at a time: all at once, they spill
     }
     float linv;
-    bf16x8 pop[2];
+    bf16x8 hi[2], lo[2];
     hide(sc, seen_bits(a, p_row, c0, j));
-    softmax8(st.m, st.l, linv, pop, sc, a.cs, VScale{1.0f, 0.0f, 1.0f, true}, [&](float x) __attribute__((always_inline)) { scale_o<D>(st, x); },
+    softmax8(st.m, st.l, linv, sc, a.cs, VScale{1.0f, 0.0f, 1.0f, true}, [&](float x) __attribute__((always_inline)) { scale_o<D>(st, x); },
              [](bool) { return 1.0f; });
-    st.l = fmaf(sum_p(pop), linv, st.l);
+    operands_p(sc, hi);
+    rest_p(sc, hi);
+    operands_p(sc, lo);
+    st.l = fmaf(sum_p(hi) + sum_p(lo), linv, st.l);
+    // o + V . P; where the product with hi alone is no number it stays (lo may be 0, or negative)
+    auto products = [&](f32x4& o, int dt, const uint32_t (&in)[2][4]) __attribute__((always_inline)) {
+        f32x4 x;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const bf16x8 v = __builtin_bit_cast(bf16x8, and4(t.v[dt * 2 + s][lane], in[s]));
+            o = mfma_bf16(v, hi[s], o);
+            x = mfma_bf16(v, lo[s], s == 0 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : x);
+        }
+        bool odd = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const bool number = fabsf(o[e]) < INFINITY;
+            odd = odd | !number;
+            o[e] = number ? o[e] + x[e] : o[e];
+        }
+        return odd;
+    };
     uint32_t in[2][4];
 #pragma unroll
     for (int s = 0; s < 2; ++s)
@@ -472,10 +510,7 @@ __device__ __forceinline__ void chunk_tail(RowState<D>& st, const TailLds<D>& t,
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) {
         o[dt] = st.o[dt];
-#pragma unroll
-        for (int s = 0; s < 2; ++s) o[dt] = mfma_bf16(__builtin_bit_cast(bf16x8, and4(t.v[dt * 2 + s][lane], in[s])), pop[s], o[dt]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) odd = odd | !(fabsf(o[dt][e]) < INFINITY);
+        odd = odd | products(o[dt], dt, in);
         if (dt & 1) __builtin_amdgcn_sched_barrier(0);
     }
     if (__builtin_expect(hidden && __builtin_amdgcn_ballot_w64(odd) != 0, 0)) {
@@ -490,9 +525,7 @@ __device__ __forceinline__ void chunk_tail(RowState<D>& st, const TailLds<D>& t,
 #pragma unroll
             for (int dt = 0; dt < D / 16; ++dt) {
                 f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int s = 0; s < 2; ++s)
-                    x = mfma_bf16(__builtin_bit_cast(bf16x8, and4(t.v[dt * 2 + s][lane], in[s])), pop[s], x);
+                products(x, dt, in);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     if (c == r) o[dt][e] = st.o[dt][e] + x[e];
@@ -691,7 +724,8 @@ __device__ __forceinline__ void chunk_completed(RowState<D>& st, const TailLds<D
     float linv;
     f16x8 pop[2];
     hide(sc, seen);
-    softmax8(st.m, st.l, linv, pop, sc, ck * scale.x, VScale{0x1p6f, 6.0f, 0x1p-6f, true}, [](float) {}, [](bool) { return 1.0f; });
+    softmax8(st.m, st.l, linv, sc, ck * scale.x, VScale{0x1p6f, 6.0f, 0x1p-6f, true}, [](float) {}, [](bool) { return 1.0f; });
+    operands_p(sc, pop);
     st.l = fmaf(sum_p(pop), linv, st.l);
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt)
@@ -1121,11 +1155,12 @@ __global__ __launch_bounds__(64 * kLoopWaves, 2) void attn8_loop_kernel(const At
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
             if (masked) hide(sc[t], seen_bits(a, row(t).p, c0, j));
-            softmax8(st[t].m, st[t].l, linv[t], pop[t], sc[t], ck[t] * ks, v,
+            softmax8(st[t].m, st[t].l, linv[t], sc[t], ck[t] * ks, v,
                      [&](float x) __attribute__((always_inline)) { scale_o<D>(st[t], x); },
                      [&](bool sees) __attribute__((always_inline)) {
                          return own_unit(k[t], sees, vs, st[0].f, largest_o<D>(st[t]), [&](int n) { shift_o<D>(st[t], n); });
                      });
+            operands_p(sc[t], pop[t]);
         }
         float sum[RT];
         __builtin_amdgcn_s_setprio(1);
