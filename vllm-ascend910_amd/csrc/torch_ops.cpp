@@ -382,7 +382,8 @@ Kv8 check_kv8(const char* op, const Tensor& k_codes, const Tensor& vt_codes, con
     const at::ScalarType dt = k_codes.scalar_type();
     TORCH_CHECK((dt == at::kChar || dt == at::kFloat8_e4m3fn) && vt_codes.scalar_type() == dt, op,
                 ": codes must be int8 or float8_e4m3fn, K and V alike");
-    TORCH_CHECK(k_codes.dim() == 5 && k_codes.size(3) == 64, op, ": k_codes must be [B, kv_heads, blocks, 64, head_dim]");
+    TORCH_CHECK(k_codes.dim() == 5 && k_codes.size(1) > 0 && k_codes.size(2) > 0 && k_codes.size(3) == 64, op,
+                ": k_codes must be [B, kv_heads, blocks, 64, head_dim], kv_heads and blocks > 0");
     const Kv8 s{k_codes.size(0), k_codes.size(1), k_codes.size(2), k_codes.size(4),
                 dt == at::kChar ? W4A8_KV_INT8 : W4A8_KV_E4M3};
     TORCH_CHECK(vt_codes.sizes() == at::IntArrayRef({s.B, s.KVH, s.NB, s.D, 64}), op,
