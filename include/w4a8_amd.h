@@ -389,7 +389,8 @@ int w4a8_rope_kv8(const void* qkv, int64_t ldq, const void* bias, const void* co
 /*
  * The cache read back: positions first .. first + n - 1 of every sequence as
  * k_out, v_out bf16 [B, KVH, n, D] -- bf16(code * scale), or the tails' values -- with
- * zeros from length[b * length_stride] (device; the positions the sequence holds) on.
+ * zeros from length[b * length_stride] (device; the positions the sequence holds, at most
+ * the L of the calls that wrote it) on.
  */
 int w4a8_kv8_read(const void* k_codes, const void* vt_codes, const void* kv_scale, const void* k_tail,
                   const void* vt_tail, int code_dtype, const void* length, int64_t length_stride, void* k_out,

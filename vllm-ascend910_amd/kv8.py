@@ -78,7 +78,9 @@ class KV8Cache:
 
     def read(self, length: torch.Tensor, first: int = 0, n: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """Positions first .. first + n - 1 as bf16 k, v [B, kv_heads, n, head_dim] (all from `first` on without
-        n), zeros from length (one, or one per sequence: the positions held) on."""
+        n), zeros from length (one, or one per sequence: the positions held, max_len where it is larger) on."""
         if n is None:
             n = self.max_len - first
+        if self.max_len % BLOCK:       # the op holds lengths to whole blocks: the last one would count as complete
+            length = length.clamp(max=self.max_len)
         return torch.ops.npu.w4a8_kv8_read(*self.tensors, length, first, n)
