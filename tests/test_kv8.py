@@ -198,3 +198,17 @@ def test_decoder_refusals(pkg, kw):
     cfg = pkg.decoder.DecoderConfig(layers=1, hidden=64, heads=1, kv_heads=1, head_dim=64, ffn=64, vocab=10, group=64)
     with pytest.raises(ValueError):
         pkg.decoder.W4A8Decoder(cfg, batch=1, max_len=8, device="cpu", **kw)
+
+
+@pytest.mark.parametrize("names,kw", [
+    (("write",), dict(B=1 << 14, T=1 << 14, KVH=2, H=2, NB=1, L=64)),        # 2^26 waves of the queries
+    (("write",), dict(B=1 << 20, T=1, KVH=8, H=8, NB=1, L=64, ldq=24 * 128)),  # 2^24 blocks of K and V
+    (("read",), dict(B=1 << 16, KVH=2, NB=64, n=4096)),
+    (("attend", "step"), dict(B=1 << 24, T=1, KVH=1, H=1, NB=1, L=64)),
+    (("attend",), dict(B=1 << 23, T=20, KVH=1, H=1, NB=1, L=64)),              # two row tiles a sequence
+])
+def test_launch_limits(lib, names, kw):
+    """Calls of 2^32 threads or more are refused by the library, before any launch."""
+    for name in names:
+        assert call(lib, name, **kw) == 5, (name, lib.w4a8_last_error())
+        assert "too many workgroups" in lib.w4a8_last_error().decode()

@@ -788,7 +788,7 @@ int w4a8_rope_kv8(const void* qkv, int64_t ldq, const void* bias, const void* co
     if (!aligned(q_out, 16)) return fail(W4A8_ERR_ALIGN, "q_out 16-byte aligned");
     // workgroups: q's, and K and V of every block a call can touch
     const int64_t blocks = std::min((T + 126) / 64, NB);
-    if ((B * T * ((H * D / 16 + 63) / 64) + 3) / 4 + B * KVH * 2 * blocks >= (1ll << 31))
+    if ((B * T * ((H * D / 16 + 63) / 64) + 3) / 4 + B * KVH * 2 * blocks > kMaxWorkgroups)
         return fail(W4A8_ERR_UNSUPPORTED, "too many workgroups for one launch: B=%lld T=%lld H=%lld", B, T, H);
     RopeKv8Args a{};
     set_kv8(a, k_codes, vt_codes, kv_scale, k_tail, vt_tail, code_dtype, NB);
@@ -822,7 +822,7 @@ int w4a8_kv8_read(const void* k_codes, const void* vt_codes, const void* kv_scal
     if (length_stride < 0) return fail(W4A8_ERR_SHAPE, "length_stride must be >= 0");
     if (!aligned(length, 8) || !aligned(k_out, 16) || !aligned(v_out, 16))
         return fail(W4A8_ERR_ALIGN, "k_out and v_out 16-byte, length 8-byte aligned");
-    if (B * KVH * 2 >= (1ll << 31) / ((n + 126) / 64))
+    if (B * KVH * 2 > kMaxWorkgroups / ((n + 126) / 64))
         return fail(W4A8_ERR_UNSUPPORTED, "too many workgroups for one launch: B=%lld KVH=%lld n=%lld", B, KVH, n);
     Kv8ReadArgs a{};
     set_kv8(a, k_codes, vt_codes, kv_scale, k_tail, vt_tail, code_dtype, NB);

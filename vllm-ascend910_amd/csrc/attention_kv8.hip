@@ -1447,7 +1447,9 @@ int64_t attention_kv8_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t K
 
 bool attention_kv8_fits(int64_t B, int64_t T, int64_t H, int64_t KVH, int64_t D, int64_t NB, int64_t window, int64_t sinks) {
     const Plan p = plan(B, T, H / KVH, KVH, D, NB, window, sinks);
-    return (B * KVH * p.ns + 7) / 8 * 8 < (1ll << 31) / p.groups && B * T < (1ll << 31) / H;
+    // the attention's workgroups, and the combine's: one a row, or one for four
+    return (B * KVH * p.ns + 7) / 8 * 8 <= kMaxWorkgroups / p.groups && B * T < (1ll << 31) / H &&
+           (p.ns == 1 || B * T * H <= kMaxWorkgroups * (p.ns > kBatch ? 1 : 4));
 }
 
 hipError_t launch_attention_kv8(const AttnKv8Args& a, hipStream_t stream) {

@@ -218,6 +218,9 @@ struct AttnArgs {
 };
 hipError_t launch_attention(const AttnArgs& a, bool split, hipStream_t stream);
 
+// A launch has fewer than 2^32 threads: workgroups of 256 (the 8-bit cache's kernels) at most.
+constexpr int64_t kMaxWorkgroups = (1ll << 24) - 1;
+
 // The 8-bit KV cache (kv8.h): NB blocks of 64 positions per pair (sequence, KV head),
 // pairs in the order b * KVH + h, every array contiguous.
 struct Kv8Cache {
