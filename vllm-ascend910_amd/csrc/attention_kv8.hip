@@ -113,8 +113,8 @@ struct VScale {
 // sum of the same rounded P, at least 1 over all of a row's positions, so with g from 2^3 on
 // a position takes at most 2^-28 from it, and as much of its own value from the product
 // (2^-13 over 32768 positions; an output's rounding is 2^-9).  f is set to bring g into
-// [2^9, 2^10): later blocks may be twice as large before O is rescaled, and 64 times as
-// small before they leave the plain way.
+// [2^9, 2^10): later blocks may be twice as large, or 64 times as small, before it is set
+// again (with O rescaled).
 constexpr float kSlack = 4.0f;
 constexpr float kLeastG = 0x1p3f, kMostG = 0x1p11f;
 
@@ -126,21 +126,24 @@ __device__ __forceinline__ int exponent(float x) { return __builtin_amdgcn_frexp
 // `rescale(x)`: O takes the factor x, a power of two; `room()`: O has no element from 2^90 on
 // (an open block's values, taken first, may be there before f is set).  f is set by the
 // first block whose scale is a number from 2^-23 on (one of zeros, or of values that small,
-// says nothing of the others) and set again, lower, where a larger one comes.  It stays in
-// [2^-32, 2^32], so that f times a sum stays inside fp32's range for rows that do not see
-// the block.
+// says nothing of the others) and set again where such a block is not plain.  It stays in
+// [2^-32, 2^30], so that f times a sum stays inside fp32's range for rows that do not see
+// the block, and rises only where O stays below 2^120: a sum of 2^25 positions with P up to
+// 2^4 and codes up to 448 is below 2^38 `most`, the largest scale before.
 template <class F, class G>
-__device__ __forceinline__ VScale v_scale(float vs, float& f, F rescale, G room) {
+__device__ __forceinline__ VScale v_scale(float vs, float& f, float& most, F rescale, G room) {
     VScale v;
-    v.g = f == 0.0f ? vs : vs * f;
-    if (f == 0.0f || v.g > kMostG) {
-        const float fn = ldexpf(1.0f, max(9 - exponent(vs), -32));
-        if (vs >= 0x1p-23f && vs < INFINITY && fn != f && (f != 0.0f || room())) {
-            rescale(f == 0.0f ? fn : fn / f);
+    v.g = vs * f;
+    if (v.g < kLeastG || v.g > kMostG) {              // (f is 0, too; as a negation of plain it spills)
+        const float was = f == 0.0f ? 1.0f : f, fn = ldexpf(1.0f, min(max(9 - exponent(vs), -32), 30));
+        v.g = vs * was;
+        if (vs >= 0x1p-23f && vs < INFINITY && fn != f && (f == 0.0f ? room() : most * fn < 0x1p82f)) {
+            rescale(fn / was);
             f = fn;
             v.g = vs * fn;
         }
     }
+    most = fmaxf(most, vs < INFINITY ? vs : 0.0f);
     v.plain = v.g >= kLeastG && v.g <= kMostG;        // false for NaN
     v.lg = __builtin_amdgcn_logf(v.g);
     v.inv = __builtin_amdgcn_rcpf(v.g);                // off by one unit in the last place at most
@@ -354,7 +357,7 @@ __device__ __forceinline__ float sum_p(const E (&pop)[2]) {
 // A wave's state over chunks of codes: its O holds f times the sum.
 template <int D>
 struct CodeState : RowState<D> {
-    float f;
+    float f, most;
 };
 
 // The state with O itself, as the tail's products, the folds and the output take it.
@@ -385,7 +388,7 @@ __device__ __forceinline__ void chunk_codes(CodeState<D>& st, const f16x8 (&qh)[
     __builtin_amdgcn_sched_barrier(0);
     next_k();
     __builtin_amdgcn_sched_barrier(0);
-    const VScale v = v_scale(vs, st.f, [&](float x) __attribute__((always_inline)) { scale_o<D>(st, x); },
+    const VScale v = v_scale(vs, st.f, st.most, [&](float x) __attribute__((always_inline)) { scale_o<D>(st, x); },
                              [&]() __attribute__((always_inline)) { return __builtin_amdgcn_ballot_w64(largest_o<D>(st) >= 0x1p90f) == 0; });
     float linv;
     f16x8 pop[2];
@@ -851,7 +854,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn8_split_kernel(const AttnKv8Ar
     uint4 q[D / 32];
     CodeState<D> st;
     state_clear(st);
-    st.f = 0.0f;
+    st.f = st.most = 0.0f;
     f16x8 qh[D / 32];
     float ck;
     const int c0 = last_chunk * kKvBlock;
@@ -1106,7 +1109,7 @@ __global__ __launch_bounds__(64 * kLoopWaves, 2) void attn8_loop_kernel(const At
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         state_clear(st[t]);
-        st[t].f = 0.0f;
+        st[t].f = st[t].most = 0.0f;
     }
     auto step = [&](const ChunkLds<D>& from, int i) __attribute__((always_inline)) {
         const int ch = vis.chunk(i), c0 = ch * kKvBlock;
@@ -1145,7 +1148,7 @@ __global__ __launch_bounds__(64 * kLoopWaves, 2) void attn8_loop_kernel(const At
             __builtin_amdgcn_sched_barrier(0);
         }
         __builtin_amdgcn_s_setprio(0);
-        const VScale v = v_scale(vs, st[0].f, [&](float x) __attribute__((always_inline)) {
+        const VScale v = v_scale(vs, st[0].f, st[0].most, [&](float x) __attribute__((always_inline)) {
 #pragma unroll
             for (int t = 0; t < RT; ++t) scale_o<D>(st[t], x);
         }, []() { return true; });                       // the open block comes last here
