@@ -70,6 +70,9 @@ struct VOps {
     uint4 v[D / 16][2];
 };
 
+// The smaller of two, NaN if either is, as vmax.
+__device__ __forceinline__ float vmin(float x, float y) { return __builtin_elementwise_minimum(x, y); }
+
 __device__ __forceinline__ int clamp_pos(int64_t p, int L) {
     return static_cast<int>(p < 0 ? 0 : (p >= L ? L - 1 : p));
 }
@@ -222,6 +225,18 @@ __device__ __forceinline__ void chunk_softmax(float& m, float& l, float& alpha, 
     }
 }
 
+// O *= alpha; nothing where no row of the wave's tile has a new maximum (alpha = 1
+// keeps every bit).
+template <int D>
+__device__ __forceinline__ void state_scale(RowState<D>& st, float alpha) {
+#pragma clang fp contract(off)
+    if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) == 0) return;
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) st.o[dt][e] = st.o[dt][e] * alpha;
+}
+
 // The softmax update and the output product of one chunk (positions c0 ..).
 template <int D>
 __device__ __forceinline__ void chunk_update(RowState<D>& st, const f32x4 (&sc)[4], const VOps<D>& vo, int c0,
@@ -315,6 +330,18 @@ __device__ __forceinline__ void rope_rotate(const uint4 (&x)[D / 32], const uint
         y[i] = make_uint4(o1[0], o1[1], o1[2], o1[3]);
         y[i + HI] = make_uint4(o2[0], o2[1], o2[2], o2[3]);
     }
+}
+
+// One bf16 of a 16-byte operand replaced (slot e of 8).
+__device__ __forceinline__ uint4 put_bf16(uint4 v, int e, uint32_t bits) {
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t lo = (e == 2 * k) ? bits : (w[k] & 0xffffu);
+        const uint32_t hi = (e == 2 * k + 1) ? bits : (w[k] >> 16);
+        w[k] = lo | (hi << 16);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // Decode launch: workgroup (split, row tile, pair) folds the chunks of its split,

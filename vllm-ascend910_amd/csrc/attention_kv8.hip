@@ -1,4 +1,4 @@
-// Grouped-query attention over the 8-bit KV cache of kv8.h (gfx950, bf16 MFMA).
+// Grouped-query attention over the 8-bit KV cache of kv8.h (gfx950, fp16 and bf16 MFMA).
 //
 // The query heads that share a KV head are the rows of one problem, as in
 // attention.hip: row r = t * G + g of pair (b, h) is head h G + g of query token t, at
@@ -763,8 +763,8 @@ __device__ __forceinline__ void write_row(uint16_t* o, const RowState<D>& st, bo
 //
 // Bound by the codes' way from memory: with the arithmetic left out (loads alone) the step
 // of 8 sequences of 28000 positions on average, 40 heads over 8 of 128 in int8 (535 MB),
-// took 91 us; it takes 90 to 100, 5.4 to 5.9 TB/s.  64 sequences of 1050 (140 MB): 29.5 us,
-// 4.8 TB/s, of which some 5 us pass before the first products and in the uneven ends.
+// took 91 us; it takes 90 to 100, 5.4 to 5.9 TB/s.  64 sequences of 1050 (140 MB): 30.0 us,
+// 4.7 TB/s, of which some 5 us pass before the first products and in the uneven ends.
 // K's loads keep the default cache policy (non-temporal ones fetched its 128-byte lines
 // twice, a wave reading half a line at a time), V's are non-temporal where one row tile
 // reads them.
@@ -948,11 +948,11 @@ __global__ __launch_bounds__(64 * NW, 2) void attn8_split_kernel(const AttnKv8Ar
 // its RT tiles.
 //
 // Bound by the vector work beside the products: 4096 tokens of 40 heads of 128 in int8
-// take 200 us (0.86 PFLOP/s), the matrix pipe busy for 36% of the cycles and the vector
-// ALU for 54% (exponentials, maxima, the conversion), nearly one after the other in a
+// take 203 us (0.85 PFLOP/s), the matrix pipe busy for 35% of the cycles and the vector
+// ALU for 55% (exponentials, maxima, the conversion), nearly one after the other in a
 // wave, with two waves a SIMD to overlap.  Without softmax and conversion the same loop
-// takes 129 us, without the softmax 168, without the conversion 182, without the matrix
-// products 206.  With two row tiles a wave the operands' way from LDS takes as long as
+// took 129 us where all of it took 200, without the softmax 168, without the conversion 182,
+// without the exponentials 193.  With two row tiles a wave the operands' way from LDS takes as long as
 // their products at the pipe's full rate; four would need 512 registers.  Tried and
 // slower: eight waves in two halves that take turns at the matrix pipe, a barrier a phase
 // (274 us); a chunk's exponentials between the products of the next (215 us).
@@ -1343,6 +1343,10 @@ struct Plan {
 // waves win where the codes take less than about 35 us.  With splits two waves serve few
 // sequences, a chunk for each wave (heads of 128, one sequence of 1000: nine splits 10.5 us,
 // five of four waves 11.7, three 11.6).
+//
+// It is made for the cache's capacity, not for what its sequences hold: 64 sequences of
+// 1000 positions take 30 us in a cache of 1024, 4096 or 16384, but 200 of 150 positions 31 us
+// in one of 192 or 4096 and 76 in one of 16384, where it splits them.
 //
 // Split kernel or loop kernel: one row tile, or two, against 64 or more rows that share
 // the conversion (40 rows over 8000 positions 24.2 / 19.5 us, 25 rows of each of 8

@@ -48,10 +48,9 @@ __device__ __forceinline__ float fold_value(float x1, float a1, float x2, float 
     return fmaf(x1, a1, x2 * a2);
 }
 
-// The larger / smaller of two, NaN if either is (v_maximum3_f32, v_minimum3_f32:
-// unlike fmaxf they need no canonicalising move per MFMA result).
+// The larger of two, NaN if either is (v_maximum3_f32: unlike fmaxf it needs no
+// canonicalising move per MFMA result).
 __device__ __forceinline__ float vmax(float x, float y) { return __builtin_elementwise_maximum(x, y); }
-__device__ __forceinline__ float vmin(float x, float y) { return __builtin_elementwise_minimum(x, y); }
 
 // The four lanes of a row (lane ^ 16, lane ^ 32) reduced by the gfx950 lane
 // swaps: x against itself gives one register holding the even and one holding
@@ -85,35 +84,11 @@ __device__ __forceinline__ void state_fold(RowState<D>& s, const RowState<D>& t)
     s.m = mn;
 }
 
-// O *= alpha; nothing where no row of the wave's tile has a new maximum (alpha = 1
-// keeps every bit).
-template <int D>
-__device__ __forceinline__ void state_scale(RowState<D>& st, float alpha) {
-#pragma clang fp contract(off)
-    if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) == 0) return;
-#pragma unroll
-    for (int dt = 0; dt < D / 16; ++dt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) st.o[dt][e] = st.o[dt][e] * alpha;
-}
-
 // x (+ bias, rounded as a bf16 add), as w4a8_rope_kv reads an input element.
 __device__ __forceinline__ float rope_in(uint32_t xbits, uint32_t bbits, bool has_bias) {
 #pragma clang fp contract(off)
     const float v = bf16_bits_to_f32(xbits);
     return has_bias ? bf16_bits_to_f32(f32_to_bf16_bits(v + bf16_bits_to_f32(bbits))) : v;
-}
-
-// One bf16 of a 16-byte operand replaced (slot e of 8).
-__device__ __forceinline__ uint4 put_bf16(uint4 v, int e, uint32_t bits) {
-    uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const uint32_t lo = (e == 2 * k) ? bits : (w[k] & 0xffffu);
-        const uint32_t hi = (e == 2 * k + 1) ? bits : (w[k] >> 16);
-        w[k] = lo | (hi << 16);
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 }  // namespace w4a8
